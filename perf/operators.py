@@ -6,7 +6,6 @@ backward   ``expert_combine_grad`` + ``expert_gather_grad``: the gradients of bo
 linear     ``linear``: residual + mul * activation(x @ W.T + bias) from the packed weights of one projection
 experts    ``expert_linear``: the same product for rows sorted by expert, each segment with its own expert's weights
 """
-import functools
 import math
 import os
 import sys
@@ -23,7 +22,6 @@ ACTIVATIONS = ("none", "relu", "relu2", "gelu", "gelu_tanh", "silu", "sigmoid")
 SHAPES = ((14336, 6144), (6144, 6144), (1536, 6144), (6144, 1536), (2304, 8192), (8192, 1024), (4096, 8192))
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "muse-bf16-proj_b200")
     if path not in sys.path:
