@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     prefetch_tmap(&p.xmap);
   }
   if (warp == 1) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kWords),
                  "r"(kTmemCols)
                  : "memory");

@@ -88,6 +88,7 @@ MBP_DEV void tc_st_a(uint32_t taddr, const uint32_t (&A)[16], int t) {
       a[2 * (2 * 2 + h) + rh] = m2;
       a[2 * (2 * 3 + h) + rh] = m3;
     }
+  __syncwarp();  // .sync.aligned: the lanes may come from branches of their own
   asm volatile(
       "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]), "r"(a[8]), "r"(a[9]),
@@ -101,6 +102,7 @@ MBP_DEV void tc_commit(uint32_t bar) {
 }
 
 MBP_DEV void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
       "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -115,6 +117,7 @@ MBP_DEV void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
 // Eight columns of the accumulator (lane = row).
 MBP_DEV void tc_ld8(uint32_t taddr, float (&v)[8]) {
   uint32_t u[8];
+  __syncwarp();
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
                : "r"(taddr));
