@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
         pr.next(kPS);
         ok = warp_wait(oempty + 8 * orr.i, orr.ph, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns);
         if (!ok) break;
+        tc_fence_after();  // the stores come after the MMAs whose commit freed the stage
         if (live) tc_st_a<false>(ta0 + (uint32_t)(orr.i * 64), A, lane & 3);
         tc_fence_before();  // the stores are complete (wait::st) and ordered before the arrive
         mbar_arrive(afull + 8 * orr.i);

@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ge
       // every load of the stage has returned before it is handed back
       mbar_arrive_dep(pempty + 8 * ps, dep);
       if (i >= kOS && !mbar_wait(oempty + 8 * as, ((i / kOS) & 1) ^ 1, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns)) break;
+      tc_fence_after();  // the stores come after the MMAs whose commit freed the stage
       if (live) tc_st_a<true>(ta0 + (uint32_t)(as * 64), A, t);
       tc_fence_before();  // the stores are complete (wait::st) and ordered before the arrive
       mbar_arrive(afull + 8 * as);

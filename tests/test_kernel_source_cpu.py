@@ -2,8 +2,6 @@
 import os
 import re
 
-import pytest
-
 from conftest import PKG_DIR
 
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -42,3 +40,15 @@ def test_masks_are_taken_by_a_converged_warp():
     """take_mask branches per lane, and matrix instructions (.sync.aligned) follow it."""
     (_, body), = functions(source("escape.cuh"), r"tgt >> lane\) & 1u")
     assert body.rstrip().endswith("__syncwarp();")
+
+
+def test_decoded_tiles_are_stored_behind_a_fence():
+    """tcgen05.st into a stage that earlier matrix products read: the wait for their commit orders the threads, and
+    tcgen05.fence::after_thread_sync orders the store behind that wait."""
+    for f in ("gemm.cu", "expert_gemm.cu"):
+        text = source(f)
+        stores = [m.start() for m in re.finditer(r"tc_st_a<", text)]
+        assert stores
+        for at in stores:
+            wait = [m.end() for m in re.finditer(r"(mbar|warp)_wait\(oempty", text[:at])][-1]
+            assert "tc_fence_after();" in text[wait:at], f
