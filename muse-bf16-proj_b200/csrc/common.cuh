@@ -140,6 +140,22 @@ MBP_DEV bool mbar_wait(uint32_t bar, uint32_t parity, int code, uint64_t limit) 
   return true;
 }
 
+struct Ring {  // position in a ring of n stages and the phase its barriers are in
+  int i;
+  uint32_t ph;
+  MBP_DEV void next(int n) {
+    if (++i == n) i = 0, ph ^= 1u;
+  }
+};
+
+// The producer of a ring, when it issues no more copies: waits until all of them have landed, so that no CTA ends while the
+// copy engine still writes to its shared memory.  Nothing to wait for after a run that met no time limit, since its consumers
+// wait for the same copies; after one that did, the limit here is the default one, whatever limit ran out.  r: the next
+// stage to fill and the phase its empty barrier is waited for with (1 in the first lap).
+MBP_DEV void drain_ring(uint32_t full, Ring r, int n, int code) {
+  for (int s = 0; s < n; ++s) mbar_wait(full + 8 * s, s < r.i ? r.ph ^ 1u : r.ph, code, kDefaultWaitLimitNs);
+}
+
 // 1-D bulk copy global -> shared through the TMA engine, completing bytes on an mbarrier.
 // dst, src 16-byte aligned; bytes a multiple of 16.
 MBP_DEV void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {

@@ -63,7 +63,7 @@ static_assert(kTmemCols == 512, "a power of two, and no more than TMEM has");
 constexpr int kX = kPS * kStage;
 constexpr int kMask = kX + kOS * 2 * kXTile;
 constexpr int kBars = kMask + kDecWarps * kMaskUnitBytes;
-constexpr int kWords = kBars + 8 * (2 * kPS + 3 * kOS + 2 * kAcc);
+constexpr int kWords = kBars + 8 * (2 * kPS + 3 * kOS + 2 * kAcc + 2);  // (one barrier more than there are: 16-byte pieces)
 constexpr int kScan = kWords + 16;
 constexpr int kTurn = kScan + 128;
 constexpr int kTable = kTurn + 4096;
@@ -82,14 +82,6 @@ struct __align__(64) ExpertParams {
   EpiArgs epi;
   GroupArgs group;
   unsigned long long wait_ns;  // limit of every bounded wait
-};
-
-struct Ring {  // position in a ring of n stages and the phase its barriers are in
-  int i;
-  uint32_t ph;
-  MBP_DEV void next(int n) {
-    if (++i == n) i = 0, ph ^= 1u;
-  }
 };
 
 // mbar_wait by a whole warp with one answer for all its lanes: what follows is warp-collective, and lanes that gave up
@@ -112,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   const uint32_t pfull = bars, pempty = pfull + 8 * kPS;
   const uint32_t afull = pempty + 8 * kPS, xfull = afull + 8 * kOS, oempty = xfull + 8 * kOS;
   const uint32_t accfull = oempty + 8 * kOS, accfree = accfull + 8 * kAcc;
+  const uint32_t done = accfree + 8 * kAcc;
   volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(sm + kWords);
   volatile uint32_t* abort_word = words + 1;  // set by the scheduler when a wait gave up
   int* scan = reinterpret_cast<int*>(sm + kScan);
@@ -133,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
       mbar_init(accfull + 8 * i, 1);
       mbar_init(accfree + 8 * i, 4);
     }
+    mbar_init(done, 1);
     *abort_word = 0u;
     fence_mbar_init();
     prefetch_tmap(&p.wmap);
@@ -234,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
           tma_load_3d(base + r.i * kStage, &p.wmap, 0, 2 * i, row, pfull + 8 * r.i);
         }
       }
+      drain_ring(pfull, r, kPS, MBP_DEV_TIMEOUT_FULL);
     }
     __syncwarp();
   } else if (warp == kXWarp) {
@@ -255,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
                           tl.tok0 + b * kBox, xfull + 8 * r.i);
         }
       }
+      drain_ring(xfull, r, kOS, MBP_DEV_TIMEOUT_FULL);
     }
     __syncwarp();
   } else if (warp == kSchedWarp) {
@@ -298,6 +294,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
       }
       acc ^= 1;
     }
+    // every issued MMA has completed before TMEM is given back, also where the epilogue gave up
+    if (lane == 0) {
+      tc_commit(done);
+      mbar_wait(done, 0, MBP_DEV_TIMEOUT_MMA, kDefaultWaitLimitNs);
+    }
+    __syncwarp();
   } else if (warp < kXWarp) {
     // ---------------- decoders: warp (d, j) = row tile d, chunk j of every stage ----------------
     // A warp may only write its TMEM lane quadrant (warp % 4): the four warps of quadrant q take row tiles 2q and

@@ -103,14 +103,6 @@ MBP_DEV bool warp_wait(uint32_t bar, uint32_t parity, int code, uint64_t limit) 
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, limit)) != 0;  // one answer for the whole warp
 }
 
-struct Ring {  // position in a ring of n stages and the phase its barriers are in
-  int i;
-  uint32_t ph;
-  MBP_DEV void next(int n) {
-    if (++i == n) i = 0, ph ^= 1u;
-  }
-};
-
 struct Chunk {
   int tt, n, nx, kci, slices;
 };
@@ -246,6 +238,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 1) k_expert_gemv(const __gr
       }
       pos += n;
     }
+    drain_ring(full, r, p.stages, MBP_DEV_TIMEOUT_FULL);
   } else {
     // ---------------- consumers: warp sl * n + wt = tile wt of a chunk's n, sl-th part of every stage's columns ----------------
     const uint32_t xr = base + L.masks + warp * L.mask;

@@ -230,19 +230,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ge
     // One box per stage: 8 row tiles x 2 sub-tiles.  A last 12-bit stage with one chunk still loads two (the
     // second belongs to the next K range, or lies past the matrix and is zero-filled); its MMAs are skipped.
     if (lane == 0) {
-      for (int i = 0; i < nst; ++i) {
+      int i = 0;
+      for (; i < nst; ++i) {
         const int ps = i % kPS;
         if (i >= kPS && !mbar_wait(pempty + 8 * ps, ((i / kPS) & 1) ^ 1, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns)) break;
         mbar_arrive_expect_tx(pfull + 8 * ps, (uint32_t)(p.wsubs * 8 * kSub));
         tma_load_3d(base + L.packed + ps * kStage, &p.wmap, 0, HILO ? 2 * (cs + i) : cs + 2 * i, rb0,
                     pfull + 8 * ps);
       }
+      drain_ring(pfull, Ring{i % kPS, (uint32_t)(i / kPS & 1) ^ 1u}, kPS, MBP_DEV_TIMEOUT_FULL);
     }
     __syncwarp();  // lanes 1-31 wait here for the producing lane
   } else if (warp == kXWarp) {
     // ---------------- x producer ----------------
     if (lane == 0) {
-      for (int i = 0; i < nst; ++i) {
+      int i = 0;
+      for (; i < nst; ++i) {
         const int xs = i % kOS;
         const int nt = HILO ? 1 : min(2, nc - 2 * i);
         if (i >= kOS && !mbar_wait(oempty + 8 * xs, ((i / kOS) & 1) ^ 1, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns)) break;
@@ -251,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ge
           tma_load_2d(base + L.x + (xs * W::kXTiles + t) * xbytes, &p.xmap, (HILO ? cs + i : cs + 2 * i + t) * 64,
                       tok0, xfull + 8 * xs);
       }
+      drain_ring(xfull, Ring{i % kOS, (uint32_t)(i / kOS & 1) ^ 1u}, kOS, MBP_DEV_TIMEOUT_FULL);
     }
     __syncwarp();
   } else if (warp == kSchedWarp) {
@@ -299,7 +303,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ge
         __syncwarp();
       }
     }
-    if (lane == 0) tc_commit(done);  // fires when every issued MMA has completed
+    if (lane == 0) {
+      tc_commit(done);  // fires when every issued MMA has completed: before TMEM is given back, also if the epilogue gave up
+      mbar_wait(done, 0, MBP_DEV_TIMEOUT_MMA, kDefaultWaitLimitNs);
+    }
     __syncwarp();
   } else {
     // ---------------- decoders: warp (d, j) = row tile d, sub-tile j of every stage ----------------

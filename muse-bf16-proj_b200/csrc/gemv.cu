@@ -153,6 +153,14 @@ struct Fmt<FMT_HILO> {
   static constexpr int UB = 2 * MBP_RAW_UNIT_BYTES;
 };
 
+// Fills i0 .. i1 - 1 of the ring have landed, under the default limit: a wait gave up, and the block must not end (nor use
+// the ring for its sums) while the copy engine still writes to its shared memory.  Off the normal path, where waiting for
+// the last copies in the producer held up the block's reduction (0.15 us a call).
+__device__ __noinline__ void await_copies(uint32_t full0, int stages, int i0, int i1) {
+  for (int i = i0; i < i1; ++i)
+    mbar_wait(full0 + 8 * (i % stages), (uint32_t)(i / stages) & 1u, MBP_DEV_TIMEOUT_FULL, kDefaultWaitLimitNs);
+}
+
 MBP_DEV void store_out(uint16_t* o, float v) { *o = __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 MBP_DEV void store_out(float* o, float v) { *o = v; }
 MBP_DEV uint32_t bf16x2_bits(float lo, float hi) {
@@ -424,7 +432,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_gemv(const __grid_constant__
     for (int it = 0; it < nit; ++it) {
       const int st = it % p.stages;
       const uint32_t ph = (uint32_t)(it / p.stages) & 1u;
-      if (it >= p.stages && !mbar_wait(empty0 + 8 * st, ph ^ 1u, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns)) break;
+      if (it >= p.stages && !mbar_wait(empty0 + 8 * st, ph ^ 1u, MBP_DEV_TIMEOUT_EMPTY, p.wait_ns)) {
+        await_copies(full0, p.stages, it - p.stages, it);
+        break;
+      }
       uint32_t bytes = 0;
       for (int q = 0; q < p.wki; ++q) {
         const int c0 = cs + q * Lk + it * p.kci, e = min(cs + (q + 1) * Lk, ce);
@@ -563,7 +574,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_gemv(const __grid_constant__
     for (int it = 0; it < nit; ++it) {
       const int st = it % p.stages;
       const uint32_t ph = (uint32_t)(it / p.stages) & 1u;
-      if (!mbar_wait(full0 + 8 * st, ph, MBP_DEV_TIMEOUT_FULL, p.wait_ns)) break;
+      if (!mbar_wait(full0 + 8 * st, ph, MBP_DEV_TIMEOUT_FULL, p.wait_ns)) {
+        await_copies(full0, p.stages, it, min(it + p.stages, nit));  // the producer may have ended: its last ring of copies
+        break;
+      }
       const unsigned char* stage = smem + st * L.sbytes;
       const int c0 = b + it * p.kci;
       const int nk = rvalid_j[0] ? max(0, min(p.kci, e - c0)) : 0;  // a warp without valid rows only drains

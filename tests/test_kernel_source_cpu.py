@@ -52,3 +52,16 @@ def test_decoded_tiles_are_stored_behind_a_fence():
         for at in stores:
             wait = [m.end() for m in re.finditer(r"(mbar|warp)_wait\(oempty", text[:at])][-1]
             assert "tc_fence_after();" in text[wait:at], f
+
+
+def test_copies_and_matrix_products_end_before_their_block():
+    """A producer whose consumers gave up leaves copies on their way into the block's shared memory: every producer waits
+    for its own, and every issuer for its products, under a limit of their own."""
+    for f, rings in (("gemm.cu", 2), ("expert_gemv.cu", 1), ("expert_gemm.cu", 2)):
+        text = source(f)
+        assert len(re.findall(r"\bdrain_ring\(", text)) == rings, f
+        if "tc_mma_ts(" in text:
+            assert re.search(r"tc_commit\(done\);\s*mbar_wait\(done, 0, \w+, kDefaultWaitLimitNs\);", text), f
+    # the GEMV waits where one of its two loops gives up
+    assert len(re.findall(r"mbar_wait\([^{]*\{\s*await_copies\(full0,[^}]*break;", source("gemv.cu"))) == 2
+    assert "kDefaultWaitLimitNs" in dict(functions(source("common.cuh"), "mbar_wait"))["drain_ring"]
