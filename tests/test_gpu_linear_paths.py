@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from helpers import weight
-from test_gpu_linear import ACTS, BF16, F32, close, expect, plan_of, rn
+from test_gpu_linear import ACTS, BF16, F32, act64, close, expect, plan_of, rn
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,30 @@ def test_half_warps_of_rows_in_the_element_wise_epilogue(tiles, act):
     close(got[:41], ref[:41], bound[:41])
     close(got[41:], *expect(x[41:], w[1], act, eb[1], None, res[41:], k))
     assert mbp.device_status() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "gelu_tanh"])
+def test_activations_where_the_exponential_leaves_the_range(act):
+    """Arguments whose e^|u| passes 2^126 and then 2^128, whose results are still above the smallest FP32 numbers.
+
+    Bound: 16 steps of the value as everywhere (for gelu_tanh the argument's own rounding too), and where e^-|u| or the result is
+    subnormal two steps of 2^-149 for the exponential and two for the quotient, which silu and gelu_tanh scale by |z|."""
+    import mbp
+    n, k = 512, 64
+    z = torch.linspace(-11.0, -9.0, n) if act == "gelu_tanh" else torch.linspace(-104.0, -80.0, n)
+    bias = z.cuda()
+    ref = act64(bias.double(), act)
+    zz = bias.double().abs()
+    u = 1.6 * (zz + 0.045 * zz ** 3) if act == "gelu_tanh" else zz
+    rel = 16 * 2.0 ** -23 + (2.0 ** -22 * u if act == "gelu_tanh" else 0)
+    bound = rel * ref.abs() + 2.0 ** -149 * 4 * (1 if act == "sigmoid" else zz + 1)
+    w = weight(2 * n, k, seed=1).view(2, n, k)
+    x = torch.zeros(70, k, dtype=BF16, device="cuda")
+    p, pe = mbp.pack_c12(w[0].contiguous()), mbp.pack_experts(w)
+    eb = torch.stack([bias, bias])
+    got = [mbp.linear(p, x[:m], bias=bias, activation=act, out_dtype=F32) for m in (5, 70)]
+    got += [mbp.expert_linear(pe, x, plan_of([30, 40], 70), bias=eb, activation=act, out_dtype=F32, tensor_cores=tc)
+            for tc in (False, True)]
+    for y in got:
+        err = (y.double() - ref).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
