@@ -9,9 +9,11 @@ File layout (little-endian):
 
     bytes 0-7       magic b"MBPPACK1"
     bytes 8-15      uint64 H, the length of the JSON header
-    bytes 16-16+H   JSON header: {"version": 1, "layers": {name: {"kind": "c12" | "hilo", "n", "k", "n_esc",
+    bytes 16-16+H   JSON header: {"version": 1 or 2, "layers": {name: {"kind": "c12" | "hilo", "n", "k", "n_esc",
                     "base_mode", "fingerprint", "arrays": {array: [offset, nbytes, dtype, shape]}}}}
-                    (a layer of experts: a c12 layer of all their rows with "experts": their number)
+                    (a layer of experts: a c12 layer of all their rows, its columns in the tensor cores' order, with
+                    "experts": their number.  A file that holds one is version 2, which readers that would take it
+                    for an ordinary matrix refuse.)
     then            each array's bytes at its offset (4096-aligned)
 
 c12 layers store ``units`` (uint8 [n/16, k/64, 1536]), ``bases`` (uint8 [n/16]), ``esc_off`` (int32
@@ -32,10 +34,11 @@ import numpy as np
 import torch
 
 from .epilogue import PackedExperts
+from .experts import MAX_EXPERTS
 from .ops import PackedC12, PackedHiLo
 
 MAGIC = b"MBPPACK1"
-VERSION = 1
+VERSION, VERSION_EXPERTS = 1, 2  # without and with layers of experts
 _ALIGN = 4096
 _DT = {"uint8": (np.uint8, torch.uint8), "int32": (np.int32, torch.int32)}
 
@@ -82,7 +85,8 @@ def save_packed(state: dict, path: str, fingerprints: dict | None = None, base_m
             blobs.append((offset, a))
             offset += -(-a.nbytes // _ALIGN) * _ALIGN
         layers[name] = meta
-    header = json.dumps({"version": VERSION, "layers": layers}).encode()
+    version = VERSION_EXPERTS if state.get("experts") else VERSION
+    header = json.dumps({"version": version, "layers": layers}).encode()
     data0 = -(-(16 + len(header)) // _ALIGN) * _ALIGN
     tmp = path + ".tmp"
     with open(tmp, "wb") as f:
@@ -102,8 +106,12 @@ def read_header(path: str) -> tuple[dict, int]:
             raise ValueError(f"{path}: not a packed weight file")
         (hl,) = struct.unpack("<Q", head[8:])
         header = json.loads(f.read(hl))
-    if header.get("version") != VERSION:
-        raise ValueError(f"{path}: format version {header.get('version')} (this build reads {VERSION})")
+    if header.get("version") not in (VERSION, VERSION_EXPERTS):
+        raise ValueError(f"{path}: format version {header.get('version')} (this build reads {VERSION} and {VERSION_EXPERTS})")
+    for name, meta in header["layers"].items():
+        e = meta.get("experts")
+        if e is not None and (meta["kind"] != "c12" or type(e) is not int or not 1 <= e <= MAX_EXPERTS or meta["n"] % (16 * e)):
+            raise ValueError(f"{path}: layer {name}: {e!r} experts of {meta['n']} rows")
     return header, -(-(16 + hl) // _ALIGN) * _ALIGN
 
 
