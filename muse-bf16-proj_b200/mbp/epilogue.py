@@ -100,7 +100,7 @@ def _epilogue(m, n, dev, bias, bias_shape, activation, mul, residual):
     return e, bias
 
 
-def _output(out, out_dtype, m, n, x, mul, residual):
+def _output(out, out_dtype, m, n, x, mul, residual, p, *others):
     """(the output tensor, its row stride)"""
     if out is None:
         if out_dtype not in _TYPES:
@@ -111,8 +111,9 @@ def _output(out, out_dtype, m, n, x, mul, residual):
     ld = check_rows(out, "out", m, n, out.dtype, x.device)
     if ld > 0x7fffffff:
         raise ValueError("out rows are too far apart")
-    if overlap(out, x):
-        raise ValueError("out overlaps x")
+    for t in (x, p.units, p.bases, p.esc_off, p.esc, *others):
+        if t is not None and overlap(out, t):
+            raise ValueError("out overlaps x, the bias, the plan or the packed weights")
     for name, t in (("mul", mul), ("residual", residual)):
         if t is not None and overlap(out, t) and not same_rows(out, t):
             raise ValueError(f"out overlaps {name} without being the same rows")
@@ -125,12 +126,12 @@ def linear(p: PackedC12, x: torch.Tensor, bias: torch.Tensor | None = None, acti
     """residual + mul * activation(x @ W[:n_out].T + bias): [m, n_out] in `out`'s type or `out_dtype` (bf16, float32).
 
     x is BF16 [m, k]; bias [n_out], mul and residual [m, n_out] (rows of any stride) are each BF16 or FP32.  `out` may
-    be `mul` or `residual` itself; any other overlap is refused."""
+    be `mul` or `residual` itself; any other overlap with an operand is refused."""
     n = p.n if n_out is None else n_out
     x = _tokens(x, p.k, p.units.device)
     m, dev = x.shape[0], x.device
     e, bias = _epilogue(m, n, dev, bias, (n,), activation, mul, residual)
-    out, ld = _output(out, out_dtype, m, n, x, mul, residual)
+    out, ld = _output(out, out_dtype, m, n, x, mul, residual, p, bias)
     e.out_f32 = out.dtype is torch.float32
     if m > GEMV_MAX_M:
         launch(dev, "mbp_gemm_c12_epi", p.desc_ptr, x.data_ptr(), m, n, ctypes.byref(e), out.data_ptr(), ld)
@@ -157,7 +158,7 @@ def expert_linear(p: PackedExperts, xs: torch.Tensor, plan: ExpertPlan, bias: to
         raise ValueError(f"xs must have the plan's {plan.src.shape[0]} rows on {plan.offsets.device}, got {rows} on {dev}")
     e, bias = _epilogue(rows, n, dev, bias, (p.experts, n), activation, mul, residual)
     new = out is None
-    out, ld = _output(out, out_dtype, rows, n, xs, mul, residual)
+    out, ld = _output(out, out_dtype, rows, n, xs, mul, residual, p.packed, bias, plan.offsets)
     e.out_f32 = out.dtype is torch.float32
     if tile:
         if tensor_cores:

@@ -89,10 +89,10 @@ def row_stride(t: torch.Tensor) -> int:
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the spans of memory of two matrices with contiguous rows meet."""
+    """Whether the spans of memory of two tensors meet."""
     def end(t):
-        return t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -161,7 +161,7 @@ def expert_gather(x: torch.Tensor, plan: ExpertPlan, out: torch.Tensor | None = 
     if new:
         out, ldo = x.new_empty((m * k, d)), d
     else:
-        ldo = _check_out(out, m * k, d, x, (x,))
+        ldo = _check_out(out, m * k, d, x, (x, plan.pos, plan.offsets))
     launch(dev, "mbp_expert_gather", x.data_ptr(), x.dtype is torch.float32, m, k, d, ldx, plan.pos.data_ptr(),
            plan.offsets.data_ptr(), plan.experts, out.data_ptr(), ldo, new)
     return out
@@ -175,7 +175,7 @@ def expert_gather_grad(dxs: torch.Tensor, plan: ExpertPlan, out: torch.Tensor | 
 def expert_combine(ys: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan, residual: torch.Tensor | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """out [m, d]: residual[t] + sum_j weights[t][j] * ys[pos[t][j]], summed in FP32 and rounded once.  Dropped
-    assignments add nothing, whatever their weight.  `out` may be `residual` itself."""
+    assignments add nothing, whatever their weight.  `out` may be `residual` itself; over any other operand it is refused."""
     return _combine(ys, _weights(weights, plan), plan, residual, out, "ys")
 
 
@@ -188,7 +188,7 @@ def _combine(ys, weights, plan, residual, out, name):
     if out is None:
         out, ldo = ys.new_empty((m, d)), d
     else:
-        ldo = _check_out(out, m, d, ys, (ys,), residual)
+        ldo = _check_out(out, m, d, ys, (ys, plan.pos) if weights is None else (ys, plan.pos, weights), residual)
     launch(dev, "mbp_expert_combine", ys.data_ptr(), dtype is torch.float32, m, k, d, ldy, plan.pos.data_ptr(),
            None if weights is None else weights.data_ptr(), None if residual is None else residual.data_ptr(), ldr,
            out.data_ptr(), ldo)
@@ -211,7 +211,7 @@ def expert_combine_grad(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Ten
     if new:
         out, ldo = ys.new_empty((m * k, d)), d
     else:
-        ldo = _check_out(out, m * k, d, ys, (ys, dout))
+        ldo = _check_out(out, m * k, d, ys, (ys, dout, weights, plan.pos, plan.offsets))
     dw = weights.new_empty((m, k))
     launch(dev, "mbp_expert_combine_grad", dout.data_ptr(), ldd, ys.data_ptr(), ldy, weights.data_ptr(),
            ys.dtype is torch.float32, m, k, d, plan.pos.data_ptr(), plan.offsets.data_ptr(), plan.experts, out.data_ptr(),

@@ -55,3 +55,38 @@ def test_activations_where_the_exponential_leaves_the_range(act):
     for y in got:
         err = (y.double() - ref).abs()
         assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def test_out_over_an_operand_is_refused():
+    """Memory that other blocks of the call still read: bias, router weights, plan, packed weights."""
+    import mbp
+    n, k, m = 64, 128, 6
+    w = weight(4 * n, k, seed=1)
+    p, pe, x = mbp.pack_c12(w[:n].contiguous()), mbp.pack_experts(w.view(4, n, k)), rn(m, k, seed=2)
+    mem = torch.zeros(m * 4 * n, dtype=F32, device="cuda")
+    out, low = mem[:m * n].view(m, n), mem.view(BF16)[:m * n].view(m, n)
+    plan = plan_of([1, 2, 0, 3], m)
+    held = mbp.ExpertPlan(mem.view(torch.int32)[:m].view(m, 1).copy_(plan.pos), plan.src,
+                          mem.view(torch.int32)[m:m + 5].copy_(plan.offsets))
+    wts = torch.ones(m, 1, device="cuda")
+    calls = [lambda: mbp.linear(p, x, bias=mem[n:2 * n], out=out), lambda: mbp.linear(p, x, bias=mem.view(BF16)[:n], out=low),
+             lambda: mbp.linear(p, x, bias=mem[m * n - 1:(m + 1) * n - 1], out=out),
+             lambda: mbp.linear(p, x, out=p.units.view(-1)[:m * n * 2].view(BF16).view(m, n)),
+             lambda: mbp.expert_linear(pe, x, plan, bias=mem[:4 * n].view(4, n), out=out),
+             lambda: mbp.expert_linear(pe, x, held, out=out),
+             lambda: mbp.expert_gather(x.float(), held, out=mem[:m * k].view(m, k)),
+             lambda: mbp.expert_combine(rn(m, n, seed=3, dtype=F32), mem[:m].view(m, 1), plan, out=out),
+             lambda: mbp.expert_combine(rn(m, n, seed=3, dtype=F32), wts, held, out=out),
+             lambda: mbp.expert_gather_grad(rn(m, n, seed=3, dtype=F32), held, out=out),
+             lambda: mbp.expert_combine_grad(rn(m, n, seed=3, dtype=F32), rn(m, n, seed=4, dtype=F32), mem[:m].view(m, 1), plan, out=out),
+             lambda: mbp.expert_combine_grad(rn(m, n, seed=3, dtype=F32), rn(m, n, seed=4, dtype=F32), wts, held, out=out)]
+    kept = mem.clone(), p.units.clone()
+    for i, f in enumerate(calls):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was not refused")
+    assert torch.equal(mem.view(torch.int32), kept[0].view(torch.int32)) and torch.equal(p.units, kept[1])
+    # the neighbours of an operand are free to be written
+    bias = mem[m * n:m * n + n]
+    ref, bound = expect(x, w[:n], "none", bias, None, None, k)
+    close(mbp.linear(p, x, bias=bias, out=out), ref, bound)
