@@ -90,3 +90,72 @@ def test_out_over_an_operand_is_refused():
     bias = mem[m * n:m * n + n]
     ref, bound = expect(x, w[:n], "none", bias, None, None, k)
     close(mbp.linear(p, x, bias=bias, out=out), ref, bound)
+
+
+@pytest.mark.parametrize("tensor_cores", [False, True])
+@pytest.mark.parametrize("borders,owners", [([0, 5, 1000, 1000, 2000], {0: (0, 5), 1: (5, 20)}),
+                                            ([-50, 5, 10, 8, 20], {0: (0, 5), 1: (5, 8), 3: (10, 20)}),
+                                            ([20, 20, 20, 20, 20], {}), ([7, 7, 3, 9, 2 ** 31 - 1], {2: (3, 9), 3: (9, 20)})])
+def test_borders_out_of_range_leave_the_neighbours_alone(tensor_cores, borders, owners):
+    """Clamped to the rows: rows of a single owner hold its product, rows outside the tensors are neither read nor written.
+    (Descending borders give a row two owners; such rows hold one of their products.)"""
+    import mbp
+    w = weight(4 * 32, 64, seed=1).view(4, 32, 64)
+    p = mbp.pack_experts(w)
+    around = torch.full((60, 64), float("nan"), dtype=BF16, device="cuda")
+    x = around[20:40]
+    x.copy_(rn(20, 64, seed=2))
+    src = torch.arange(20, dtype=torch.int32, device="cuda")
+    plan = mbp.ExpertPlan(src.view(20, 1), src, torch.tensor(borders, dtype=torch.int32, device="cuda"))
+    buf = torch.full((60, 40), 7.0, device="cuda")
+    mbp.expert_linear(p, x, plan, out=buf[20:40, 4:36], tensor_cores=tensor_cores)
+    for e, (a, b) in owners.items():
+        close(buf[20 + a:20 + b, 4:36], *expect(x[a:b], w[e], "none", None, None, None, 64))
+    assert not bool(torch.isnan(buf).any())
+    if not owners:
+        assert bool((buf == 7.0).all())
+    buf[20:40, 4:36] = 7.0
+    assert bool((buf == 7.0).all())
+    assert mbp.device_status() == 0
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [5, 70])
+def test_each_activation_within_its_own_bound(act, m):
+    """Arguments from -60 to 60, FP32.  none and relu are exact, relu2 is one rounding.  gelu: the argument of erfc carries
+    two roundings, each of which moves erfc(a) by 2 a^2 = z^2 times as much, and 16 steps for erfc itself and the products;
+    silu and sigmoid 16 steps; gelu_tanh those and the roundings of its argument u = 1.6 (z + 0.045 z^3), four at most.
+    Where the exponential or erfc is subnormal, 4 steps of 2^-149, scaled by |z|."""
+    import mbp
+    z = torch.linspace(-60, 60, 512, device="cuda")
+    p = mbp.pack_c12(weight(512, 64, seed=7))
+    got = mbp.linear(p, torch.zeros(m, 64, dtype=BF16, device="cuda"), bias=z, activation=act, out_dtype=F32)
+    zd = z.double()
+    ref, step = act64(zd, act), 2.0 ** -23
+    u = 1.6 * (zd.abs() + 0.045 * zd.abs() ** 3)
+    rel = {"none": 0.0, "relu": 0.0, "relu2": step / 2, "gelu": (zd ** 2 + 16) * step, "gelu_tanh": (2 * u + 16) * step}.get(act, 16 * step)
+    bound = rel * ref.abs() + (0 if act in ("none", "relu") else 2.0 ** -149 * 4 * (zd.abs() + 1))
+    err = (got.double() - ref).abs()
+    assert bool((err <= bound).all()), float((err - bound).max())
+
+
+@pytest.mark.parametrize("m", [1, 16, 300])
+def test_as_many_experts_as_the_router_has(m):
+    """256 experts of 1536 x 6144, 8 for each token: the router's own widths, on both kernels."""
+    import mbp
+    e, n, k = 256, 1536, 6144
+    base = weight(n, k, seed=5)
+    scale = 2.0 ** (torch.arange(e, device="cuda") % 5 - 2)  # exact in BF16, so that the experts differ
+    w = base.unsqueeze(0) * scale.view(e, 1, 1).to(BF16)
+    p = mbp.pack_experts(w)
+    g = torch.Generator(device="cuda").manual_seed(m)
+    ids = torch.randn(m, e, generator=g, device="cuda").topk(8, dim=1).indices.to(torch.int32)
+    plan = mbp.expert_sort(ids, e)
+    x = rn(m, k, seed=m)
+    xs = mbp.expert_gather(x, plan)
+    owner = ids.reshape(-1)[plan.src.long()].long()
+    ref, bound = expect(xs, base, "none", None, None, None, k)
+    ref, bound = ref * scale[owner].view(-1, 1), bound * scale[owner].view(-1, 1)
+    for kw in ({}, {"tensor_cores": False}, {"tensor_cores": True}):
+        close(mbp.expert_linear(p, xs, plan, **kw), ref, bound)
+    assert mbp.device_status() == 0
