@@ -109,7 +109,7 @@ struct EscCursor {
   }
 };
 
-// Loads (and re-zeroes) this lane's two mask words of a unit mask when the lane was targeted.  The whole warp calls it.
+// Loads (and re-zeroes) this lane's two mask words of a unit mask when the lane was targeted.
 MBP_DEV void take_mask(uint32_t mask, uint32_t tgt, int lane, uint4& m0, uint4& m1) {
   if ((tgt >> lane) & 1u) {
     const uint32_t a = mask + (uint32_t)lane * 16u;
@@ -121,7 +121,6 @@ MBP_DEV void take_mask(uint32_t mask, uint32_t tgt, int lane, uint4& m0, uint4& 
     m0 = make_uint4(0, 0, 0, 0);
     m1 = make_uint4(0, 0, 0, 0);
   }
-  __syncwarp();  // matrix instructions and TMEM stores (.sync.aligned) follow
 }
 
 // Zeroes `bytes` (multiple of 512) of masks starting at `mask`, one warp.

@@ -291,7 +291,10 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 1) k_expert_gemv(const __gr
         for (int j = 0; j < J; ++j)
 #pragma unroll
           for (int l = 0; l < 3; ++l) u[j][l] = lds128(stage + uoff + (uint32_t)((k0 + j) * kSub + l * 512));
-        if constexpr (ESC) take_mask(xr, tgt, lane, m0, m1);
+        if constexpr (ESC) {
+          take_mask(xr, tgt, lane, m0, m1);
+          __syncwarp();  // a branch per lane, and ldmatrix and mma.sync are .sync.aligned
+        }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           uint32_t bx[MT][8];

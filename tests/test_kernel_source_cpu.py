@@ -36,10 +36,10 @@ def test_warp_collective_tmem_accesses_reconverge_first():
         assert not re.search(r"tcgen05\.(ld|st)\.", text)  # only through the helpers
 
 
-def test_masks_are_taken_by_a_converged_warp():
-    """take_mask branches per lane, and matrix instructions (.sync.aligned) follow it."""
-    (_, body), = functions(source("escape.cuh"), r"tgt >> lane\) & 1u")
-    assert body.rstrip().endswith("__syncwarp();")
+def test_escape_masks_in_front_of_matrix_instructions():
+    """take_mask branches per lane; ldmatrix and mma.sync (.sync.aligned) follow it in the expert GEMV, tcgen05.st behind
+    tc_st_a's own __syncwarp in the tensor-core kernels."""
+    assert re.search(r"take_mask\([^;]*\);\s*__syncwarp\(\);", source("expert_gemv.cu"))
 
 
 def test_decoded_tiles_are_stored_behind_a_fence():
