@@ -12,15 +12,16 @@
 // stages to the issuing thread); what differs:
 //   * every ring and its phases run on across the tiles, so the next tile's weights and x are on their way while
 //     this one ends; the epilogue has four warps of its own (one per TMEM lane quadrant) and the accumulator is
-//     double-buffered, so the decoders and the MMAs go on meanwhile.  (One CTA
-//     per tile, as the projection GEMM runs, left each SM idle for ~5 us between tiles; decoders that also ran the
-//     epilogue needed more registers than they have and took 1.4 times as long per stage.)
+//     double-buffered, so the decoders and the MMAs go on meanwhile;
 //   * the MMA's N and the x boxes (32 rows each) follow the tile's own row count;
 //   * the weights are packed in the tensor cores' pair order (mbp_expert_order), so decoded registers go to TMEM
 //     without the quad transpose.
-// Bound: up to ~64 rows per expert the MMA's A operand in TMEM (~145 cycles an MMA whatever its N, so ~0.62 us a stage of
-// 24.5 KB: 40 GB/s an SM, near HBM's rate over all SMs), then the L2 -> SM traffic of x, which every row block reads
-// again.  64 experts of 1536 x 6144 (906 MB): 190 us at 8 rows each (5.2 rounds of tiles take 6), 272 us at 128 rows.
+// Bound: the chain of a stage, not a unit.  12 experts of 1536 x 6144 (one round of tiles), 8 / 128 rows each: 44 / 59 us,
+// DRAM 3.9 / 3.2 TB/s, ALU pipe 51 / 42 % of its cycles (the decode), tensor pipe 4 / 25 %, L2 to SM 15 / 20 %; warps wait for
+// loads and barriers.  A stage of 24.5 KB of weights is a load, a decode, a store to TMEM, a hand-over, eight MMAs and a
+// commit; with 128 rows its 32 KB of x, which every row block reads again, have to arrive as well.  64 experts (906 MB; 5.2
+// rounds of tiles take 6): 195 us at 8 rows each, 216 at 64, 262 at 128, 399 at 160 (two token tiles: the weights decoded
+// twice).  ptxas spills 24 bytes of the 80 registers that 768 threads leave each.
 // All waits are bounded; TMEM is always released.
 #include <cstdlib>
 #include <map>

@@ -10,11 +10,10 @@
 // adds their sums in order.  The producer warp's ring runs on across the chunks, so HBM keeps busy through an epilogue.
 // The weights are packed in the tensor cores' pair order (mbp_expert_order), so the B fragments are ldmatrix loads of x
 // as it is.
-// Bound: HBM.  64 experts of 1536 x 6144, 8 of them per token, 1 / 4 / 8 / 30 tokens: 24 / 49 / 85 / 135 us (floors of the
-// used experts' bytes at the measured copy rate 17 / 44 / 78 / 115; a grid of one block per part of an expert took 25 / 75 /
-// 114 / 151).  One token of 2 experts gives a third of the SMs two tiles and the rest one: 13.2 us against 10.7 for that grid,
-// which could split K over a cluster's blocks.  Two experts of 512 x 1024: 6.3 us, 0.9 us more than that grid: a longer way
-// to the first load and the partial sums' way through shared memory.
+// Bound: HBM.  64 experts of 1536 x 6144, 8 of them per token, 1 / 8 / 30 tokens: 24 / 86 / 139 us (floors of the used
+// experts' bytes at the measured copy rate 17 / 78 / 115).  Few tiles leave SMs idle: one token of 2 experts gives a third of
+// them two tiles and the rest one, 13.2 us; two experts of 512 x 1024 take 6.3 us, mostly the way to the first load and the
+// partial sums' way through shared memory.
 // All waits are bounded and reported through the device status word.
 #include <cstdlib>
 #include <map>

@@ -877,7 +877,7 @@ int max_ctas(KernelFn fn, int split, int threads, int smem) {
 //   * each level of cluster split-K costs a fixed reduction / synchronisation overhead;
 //   * ~8 consumer warps per SM (fewer, fatter CTAs when the token tile is large and 2 CTAs fit an SM).
 // Only single-wave launches are considered.
-// zb: token blocks (grid z); outk: the output kind of the launched instance.
+// zb: token blocks (grid z); outk: MBP_OUT_BF16 or MBP_OUT_F32 (an epilogue runs in the geometry of its output type).
 int plan_search(int fmt, int Rout, int C, int mt, int zb, int outk, bool esc, mbp_gemv_geom* g) {
   constexpr double kHbmBw = 6.0e12, kSmBw = 45.0e9, kSplitCost = 1.2e-6;
   const int ub = ub_of(fmt);

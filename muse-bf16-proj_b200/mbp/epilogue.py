@@ -18,7 +18,9 @@ from .experts import ExpertPlan, check_rows, launch, overlap, same_rows
 from .ops import BASE_TILE, PackedC12, _check_x, pack_c12, unpack_c12
 
 ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5, "sigmoid": 6}  # MBP_ACT_*
-GEMV_MAX_M = 32  # one matrix: the GEMV up to 32 tokens, the tcgen05 GEMM above (the boundary of kernel_fn)
+# One matrix: the GEMV up to 32 tokens, the tcgen05 GEMM above, the boundary of kernel_fn (so that both give the same bits).
+# A small matrix would take the GEMM earlier: 1536 x 6144 at 24 tokens 17 us on the GEMV and 11 us there.
+GEMV_MAX_M = 32
 _TYPES = (torch.bfloat16, torch.float32)
 
 
@@ -176,8 +178,10 @@ def expert_linear(p: PackedExperts, xs: torch.Tensor, plan: ExpertPlan, bias: to
 
 
 def _use_tensor_cores(rows: int, p: PackedExperts) -> bool:
-    """Measured, GEMV / GEMM in us: 64 experts at 8 and 10 rows per expert 161 / 163 and 170 / 164 (1536 x 6144), 174 / 184
-    and 191 / 185 (6144 x 1536); 64 experts of 512 x 1024, whose 50 MB the GEMV streams in less than the GEMM's fixed cost,
-    16.3 / 20.5 at 12 and 21.4 / 21.0 at 16."""
+    """Measured, GEMV / GEMM in us.  Selections with popular and unused experts, 64 of them: at 8 and 10 rows per expert on
+    average 161 / 163 and 170 / 164 (1536 x 6144), 174 / 184 and 191 / 185 (6144 x 1536); of 512 x 1024, whose 50 MB the GEMV
+    streams in less than the GEMM's fixed cost, 16.3 / 20.5 at 12 and 21.4 / 21.0 at 16.  As many rows for each: 64 of
+    1536 x 6144 153 / 195 at 8 and 177 / 196 at 12, 256 of them 601 / 675 and 702 / 682.  Not measured: a few experts, and
+    one that takes most of the rows."""
     per = 16 if p.packed.n * p.k <= 64 << 20 else 8
     return rows > per * p.experts

@@ -9,8 +9,10 @@ logits).
     out = mbp.expert_combine(ys, w, plan, residual=x)   # [m, d]
 
 and, for training, ``expert_combine_grad`` and ``expert_gather_grad``.  Rows are BF16 or FP32, sums FP32; every call
-is one launch on the current stream of the tensors' device, allocates nothing but its outputs, uses no atomics
-(repeated calls give identical bits) and can be captured in a CUDA graph.
+is one launch on the current stream of the tensors' device, uses no atomics (repeated calls give identical bits), needs no
+workspace and can be captured in a CUDA graph.  Router weights and ids whose strides the kernels do not take are copied
+first.  The gradients are those of the row movements; the products in between have none here (their weights are packed for
+serving): a program that trains the experts brings its own product from dys to dxs.
 """
 from __future__ import annotations
 
